@@ -1,0 +1,58 @@
+"""
+What the GPU code of this repository may hold, checked over its sources: the kernels, the headers they include, the probes
+under tools/ and every script that could build one.
+"""
+
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE_DIRS = ('nufhe_amd', 'nufhe', 'include', 'tools', 'examples', 'oracle', 'tests')
+SOURCE_TYPES = ('.hip', '.h', '.hpp', '.c', '.cpp', '.s', '.S', '.py', '.sh')
+
+# stores and atomics of the scalar unit, and that cache's write-back and discard
+SCALAR_WRITE = re.compile(r'\bs_(?:(?:buffer_|scratch_)?store_|(?:buffer_)?atomic_|dcache_(?:wb|discard))')
+
+
+def sources():
+    for top in SOURCE_DIRS:
+        for where, dirs, files in os.walk(os.path.join(ROOT, top)):
+            dirs[:] = [d for d in dirs if d not in ('__pycache__', 'build', '_ref')]
+            for name in files:
+                if name.endswith(SOURCE_TYPES) or name == 'Makefile':
+                    yield os.path.join(where, name)
+
+
+def hits(pattern):
+    found = []
+    for path in sources():
+        with open(path, errors='replace') as f:
+            for number, line in enumerate(f, 1):
+                if pattern.search(line):
+                    found.append('%s:%d: %s' % (os.path.relpath(path, ROOT), number, line.strip()))
+    return found
+
+
+def test_the_scan_reaches_the_kernels():
+    names = {os.path.relpath(p, ROOT) for p in sources()}
+    assert {'nufhe_amd/csrc/kernels.hip', 'nufhe_amd/csrc/api.hip', 'nufhe_amd/csrc/Makefile',
+            'tools/microbench_issue.hip', 'tools/build_variant.sh'} <= names
+
+
+@pytest.mark.parametrize('op', ['store_dword', 'store_dwordx4', 'buffer_store_dword', 'scratch_store_dword', 'atomic_add',
+                                'buffer_atomic_add', 'dcache_wb', 'dcache_wb_vol', 'dcache_discard'])
+def test_the_pattern_knows_the_scalar_writes(op):
+    assert SCALAR_WRITE.search('asm volatile("s_%s s0, s[2:3], 0")' % op)
+
+
+@pytest.mark.parametrize('op', ['load_dwordx2', 'buffer_load_dword', 'dcache_inv', 'waitcnt'])
+def test_the_pattern_leaves_the_reads_alone(op):
+    assert not SCALAR_WRITE.search('asm volatile("s_%s s0, s[2:3], 0")' % op)
+
+
+def test_no_write_through_the_scalar_data_cache():
+    """GPU memory is written with vector stores: nothing writes the scalar data cache back on its own, and the unit's own
+    write-back is no part of this code."""
+    assert hits(SCALAR_WRITE) == []
