@@ -1036,6 +1036,15 @@ __global__ __launch_bounds__(64) void k_write_table(uint4 *__restrict__ dst, Tab
     for (int i = threadIdx.x; i < words; i += 64) dst[i] = c.w[i];
 }
 
+// Clears words, grid-stride: the accumulators k_keyswitch_a adds into (2 KB - 1 MB below the matrix-core kernel's first size:
+// bound by the launch, not by the bytes).  A kernel of its own because gate calls are captured into graphs, where a memset
+// node can give wrong words on replays after the first.
+#define ZERO_MAX_BLOCKS 4096
+__global__ __launch_bounds__(256) void k_zero_words(u32 *__restrict__ dst, long count)
+{
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) dst[i] = 0;
+}
+
 // Heterogeneous gate batch, step 1: the linear pre-combination of every gate of the batch (gates.py:104-110 and
 // siblings: (0, c) + pa a + pb b, int32 wraparound) into the rows of ONE LWE(n) array, so that a single bootstrap launch
 // covers independent gates of different kinds.  One work-group per row.
@@ -1871,7 +1880,11 @@ hipError_t launch_keyswitch(const KsLaunch &P, const KsFinal &F, hipStream_t str
         hipLaunchKernelGGL(k_keyswitch_finalize, dim3((unsigned)P.nbits), dim3(256), 0, stream, F);
         return hipGetLastError();
     }
-    e = hipMemsetAsync(P.acc, 0, (size_t)P.nbits * P.n * sizeof(u32), stream);
+    const long words = P.nbits * (long)P.n;
+    const long zero_blocks = (words + 255) / 256;
+    hipLaunchKernelGGL(k_zero_words, dim3((unsigned)(zero_blocks < ZERO_MAX_BLOCKS ? zero_blocks : ZERO_MAX_BLOCKS)), dim3(256), 0,
+                       stream, P.acc, words);
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid(blocks_for(P.nbits, KS_TILE_BITS), P.input_size / P.j_per_block);
     hipLaunchKernelGGL(k_keyswitch_a, grid, dim3(KS_BLOCK_THREADS), KS_LDS_BYTES, stream, P);

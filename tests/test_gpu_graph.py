@@ -129,3 +129,82 @@ def test_captured_chain_on_the_exact_engine(side_stream_env):
             assert out == expect
             assert (ctx.decrypt(secret2, out) == numpy.where(~(ms2[0] & ms2[1]), ms2[2], ms2[0])).all()
             g.close()
+
+
+def node_types(raw_graph):
+    """The kinds of a captured graph's nodes (hipGraphNodeType), read through the HIP library the kernels are linked with."""
+    import ctypes
+    from nufhe_amd import _lib
+    hip = _lib.lib()
+    count = ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(ctypes.c_void_p(raw_graph), None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert hip.hipGraphGetNodes(ctypes.c_void_p(raw_graph), nodes, ctypes.byref(count)) == 0
+    types = []
+    for node in nodes:
+        kind = ctypes.c_int(-1)
+        assert hip.hipGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        types.append(kind.value)
+    return types
+
+
+@pytest.mark.parametrize('engine', ['native', 'exact-fft'])
+@pytest.mark.parametrize('bits', [1, 37, 600])
+def test_captured_gates_are_kernel_nodes_only(side_stream_env, monkeypatch, bits, engine):
+    """A memset node of a captured graph can give wrong words on replays after the first, so every node a gate records is
+    a kernel -- below the matrix-core keyswitch's first size (1 and 37 bits: the accumulators are cleared by a kernel of
+    the library) and above it (600).  Every one of several replays equals the eager words, with eager gates of another
+    size, which use the same scratch, and a synchronization in between."""
+    import torch
+    import nufhe_amd as nufhe
+    e = side_stream_env
+    ctx, vm, secret, cloud, stream, thr = e['ctx'], e['vm'], e['secret'], e['cloud'], e['stream'], e['thr']
+    rs = numpy.random.RandomState(100 + bits)
+    graph_class = torch.cuda.CUDAGraph
+    monkeypatch.setattr(torch.cuda, 'CUDAGraph', lambda: graph_class(keep_graph=True))
+    with torch.cuda.stream(stream):
+        cloud.set_engine(engine)
+        try:
+            cs = [ctx.encrypt(secret, rs.randint(0, 2, bits).astype(bool)) for _ in range(3)]
+            other = [ctx.encrypt(secret, rs.randint(0, 2, 50).astype(bool)) for _ in range(2)]
+
+            def circuit():
+                return vm.gate_mux(vm.gate_nand(cs[0], cs[1]), cs[2], cs[0])
+            g = nufhe.GateGraph(thr)
+            out = g.capture(circuit)
+            assert set(node_types(g.graph.raw_cuda_graph())) == {0}           # hipGraphNodeTypeKernel
+            for _ in range(4):
+                for c in cs:
+                    c[...] = ctx.encrypt(secret, rs.randint(0, 2, bits).astype(bool))
+                expect = circuit()
+                vm.gate_xor(other[0], other[1])
+                thr.synchronize()
+                g.replay()
+                thr.synchronize()
+                assert out == expect
+            g.close()
+        finally:
+            cloud.set_engine('native')
+
+
+@pytest.mark.parametrize('bits', [1, 513, 2600])
+def test_lds_window_keyswitch_clears_its_accumulators(side_stream_env, bits):
+    """The keyswitch without matrix cores adds into accumulators that hold the words of the gate before: two gates on other
+    inputs in a row, at sizes where the clearing kernel has one block, many, and more words than threads (2600 bits),
+    give the words of the matrix-core kernel, which writes every word once."""
+    import torch
+    from nufhe_amd import _lib
+    e = side_stream_env
+    ctx, vm, secret, stream, thr = e['ctx'], e['vm'], e['secret'], e['stream'], e['thr']
+    rs = numpy.random.RandomState(bits)
+    with torch.cuda.stream(stream):
+        cs = [ctx.encrypt(secret, rs.randint(0, 2, bits).astype(bool)) for _ in range(3)]
+        words = {}
+        try:
+            for mode in (0, 2):
+                _lib.call('nufhe_ctx_set_keyswitch_mfma', thr.handle, mode)
+                words[mode] = [vm.gate_nand(cs[0], cs[1]), vm.gate_xor(cs[1], cs[2])]
+        finally:
+            _lib.call('nufhe_ctx_set_keyswitch_mfma', thr.handle, 1)
+        assert words[0][0] == words[2][0] and words[0][1] == words[2][1]
+        assert not (words[0][0] == words[0][1])
