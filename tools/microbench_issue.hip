@@ -39,7 +39,6 @@ __device__ __forceinline__ void body(uint32_t (&a)[16], uint64_t (&w)[8], uint32
         else if (OP == 13) A1("v_fma_f32 %0, %0, %1, %2");
         else if (OP == 14) A1("v_fmac_f32 %0, %1, %2");
         else if (OP == 15) asm volatile("v_fma_f64 %0, %0, %0, %0" : "+v"(w[i % (CH > 8 ? 8 : CH)]));
-        else if (OP == 16) asm volatile("v_pk_fma_f32 %0, %0, %0, %0" : "+v"(w[i % (CH > 8 ? 8 : CH)]));
         else if (OP == 17) A1("v_mul_lo_u32 %0, %0, %1");
         else if (OP == 18) A1("v_mul_u32_u24 %0, %0, %1");
         else if (OP == 19) A1("v_mad_u32_u24 %0, %0, %1, %2");
@@ -332,7 +331,6 @@ int main(int argc, char **argv)
     run_op<31>("v_dot4_i32_i8", d_out, d_cyc);
     run_op<13>("v_fma_f32", d_out, d_cyc);
     run_op<14>("v_fmac_f32", d_out, d_cyc);
-    run_op<16>("v_pk_fma_f32", d_out, d_cyc);
     run_op<15>("v_fma_f64", d_out, d_cyc);
     run_op<29>("blend 3 add : 2 lshl_add", d_out, d_cyc);
     run_op<60>("v_cvt_f64_i32", d_out, d_cyc);
