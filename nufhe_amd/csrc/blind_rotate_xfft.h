@@ -76,7 +76,7 @@ FF_FN u32 xfft_round_lo32(double v)
 // The ~27 lane-dependent LDS addresses of the exchanges are loop invariants that the compiler keeps in registers across
 // the product phases (and partly spills).  Re-deriving the lane record from an opaque copy of the lane index in front of
 // every transform group makes them phase-local: ~30 more integer instructions per group, ~25 registers free while the
-// key loads are in flight (256 VGPRs + 56 B scratch -> 252, none).
+// key loads are in flight (256 VGPRs + 56 B scratch -> 243, none).
 FF_FN FftLane brx_fresh_lane(const FftLane &L)
 {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -5,6 +5,8 @@ under tools/ and every script that could build one.
 
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 
@@ -73,3 +75,60 @@ def test_the_pattern_leaves_the_16_bit_packed_arithmetic_alone(op):
 
 def test_no_packed_fp32_arithmetic_by_hand():
     assert hits(PACKED_FP32) == []
+
+
+NO_PACKED_FP32 = '-Xclang -target-feature -Xclang -packed-fp32-ops'
+
+
+def library_compiles(*make_args):
+    """the compile commands `make` would run for the library's objects"""
+    text = subprocess.run(['make', '-n'] + list(make_args), cwd=os.path.join(ROOT, 'nufhe_amd', 'csrc'), text=True, check=True,
+                          capture_output=True).stdout
+    return [l for l in text.split('\n') if ' -c ' in l]
+
+
+def test_every_object_is_compiled_without_packed_fp32():
+    lines = library_compiles('-B')
+    assert len(lines) == 5 and all(NO_PACKED_FP32 in l for l in lines)
+
+
+def test_other_flags_make_other_objects(tmp_path):
+    """An object that is older than the Makefile is compiled again: it may have been made with other flags."""
+    csrc = tmp_path / 'nufhe_amd' / 'csrc'
+    shutil.copytree(os.path.join(ROOT, 'nufhe_amd', 'csrc'), csrc, ignore=shutil.ignore_patterns('*.o'))
+    shutil.copytree(os.path.join(ROOT, 'include'), tmp_path / 'include')
+    objects = ['kernels.o', 'kernels_team8.o', 'kernels_team.o', 'kernels_xfft.o', 'api.o']
+    for name in objects:
+        (csrc / name).touch()
+    times = {name: 2000 for name in objects}
+    for makefile, compiled in ((1000, 0), (3000, len(objects))):
+        times['Makefile'] = makefile
+        for path in list(csrc.iterdir()) + list((tmp_path / 'include').iterdir()):
+            os.utime(path, (times.get(path.name, 1000),) * 2)
+        out = subprocess.run(['make', '-n'] + objects, cwd=csrc, text=True, check=True, capture_output=True).stdout
+        assert sum(' -c ' in l for l in out.split('\n')) == compiled
+
+
+def test_scripts_compile_without_packed_fp32_too():
+    """The tools that build variants of the library, read its ISA or say how a probe is built."""
+    for path in sources():
+        with open(path, errors='replace') as f:
+            text = f.read()
+        if os.path.basename(os.path.dirname(path)) == 'tools' and re.search(r"hipcc\b.*offload-arch|hipcc \$FLAGS", text):
+            assert NO_PACKED_FP32 in text or NO_PACKED_FP32.replace(' ', "', '") in text, path
+
+
+def test_the_flags_keep_packed_fp32_out_of_the_isa(tmp_path):
+    """Float code that the compiler would pair by itself: packed arithmetic without the flags, none with the library's."""
+    src = tmp_path / 'pairs.hip'
+    src.write_text('#include <hip/hip_runtime.h>\n'
+                   '__global__ void k(float2 *x, float2 a, float2 b)\n'
+                   '{ float2 v = x[threadIdx.x]; v.x = v.x * a.x + b.x; v.y = v.y * a.y + b.y; x[threadIdx.x] = v; }\n')
+    with_flags = library_compiles('-B')[0].split(' -c ')[0].split()
+    plain = [w for w in with_flags if w not in NO_PACKED_FP32.split()]
+    found = {}
+    for name, cmd in (('flags', with_flags), ('plain', plain)):
+        out = tmp_path / (name + '.s')
+        subprocess.check_call(cmd + ['--cuda-device-only', '-S', str(src), '-o', str(out)], stderr=subprocess.DEVNULL)
+        found[name] = bool(PACKED_FP32.search(out.read_text()))
+    assert found == {'flags': False, 'plain': True}

@@ -6,7 +6,7 @@ NAME=$1; shift
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 mkdir -p "$ROOT/gpurun_variants/obj_$NAME"
 cd "$ROOT/nufhe_amd/csrc"
-FLAGS="-O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -Wno-pass-failed -Wno-unused-value $@"
+FLAGS="-O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-function -Wno-pass-failed -Wno-unused-value $@"
 /opt/rocm/bin/hipcc $FLAGS -c kernels.hip -o "$ROOT/gpurun_variants/obj_$NAME/kernels.o" -Rpass-analysis=kernel-resource-usage 2> "$ROOT/gpurun_variants/obj_$NAME/kernels.log" &
 /opt/rocm/bin/hipcc $FLAGS -c api.hip -o "$ROOT/gpurun_variants/obj_$NAME/api.o" &
 /opt/rocm/bin/hipcc $FLAGS ${TEAM8_FLAGS--mllvm -amdgpu-sched-strategy=max-ilp -DFF_MULWIDE_PLAIN} -c kernels_team8.hip -o "$ROOT/gpurun_variants/obj_$NAME/kernels_team8.o" &

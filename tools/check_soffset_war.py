@@ -49,6 +49,7 @@ def main():
     for unit, flags in UNITS.items():
         asm = '/tmp/war_%s.s' % unit.replace('.hip', '')
         subprocess.check_call(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', '-S', '--cuda-device-only',
+                               '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
                                unit, '-o', asm] + flags, cwd=CSRC, stderr=subprocess.DEVNULL)
         lines = open(asm).read().split('\n')
         nbuf = sum(1 for l in lines if re.match(r'\s+buffer_', l))

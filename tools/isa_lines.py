@@ -47,6 +47,7 @@ def main():
     src = os.path.abspath(pos[1]) if len(pos) > 1 else os.path.join(CSRC, unit)
     asm = '/tmp/nufhe_kernels_g.s'
     out = subprocess.run(['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-S', '--cuda-device-only', '-I' + CSRC,
+                          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
                           '-gline-tables-only', src, '-o', asm] + [a for a in sys.argv[1:] if a.startswith('-D')],
                          cwd=CSRC, capture_output=True, text=True)
     if out.returncode:

@@ -120,6 +120,7 @@ def main():
             asm = '/tmp/nufhe_%s.s' % src.replace('.hip', '')
             out = subprocess.run(
                 ['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-S', '--cuda-device-only', src, '-o', asm,
+                 '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
                  '-Rpass-analysis=kernel-resource-usage'] + args, cwd=CSRC, capture_output=True, text=True)
             if out.returncode:
                 sys.exit(out.stderr[-3000:])

@@ -2,7 +2,7 @@
 // built from.  Every instruction is emitted through inline asm (the compiler cannot fold the
 // loop), 16 independent chains per lane, 8 waves per SIMD.  Reports cycles per wave-instruction
 // per SIMD (at the clock measured with s_memtime-free wall time / assumed 2.4 GHz).
-// Build: hipcc --offload-arch=gfx950 -O3 microbench.hip -o microbench
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops microbench.hip -o microbench
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

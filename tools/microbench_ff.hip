@@ -3,7 +3,7 @@
 //   ASM: EXEC-predicated correction (s_and_saveexec / one VALU add / restore): fewer VALU issues,
 //        the mask bookkeeping moves to the scalar unit
 // 2 waves per SIMD (256 blocks x 512 threads), CHAINS independent dependency chains per lane.
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -I../nufhe_amd/csrc microbench_ff.hip -o microbench_ff
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -I../nufhe_amd/csrc microbench_ff.hip -o microbench_ff
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

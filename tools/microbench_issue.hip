@@ -7,7 +7,7 @@
 // cycles per wave-instruction per SIMD = (wave-resident ticks) / (instructions of ONE wave) / (waves per SIMD).
 // A second pass uses ONE dependent chain (CHAINS = 1): the back-to-back issue latency of a single wave.
 //
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 microbench_issue.hip -o microbench_issue
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 microbench_issue.hip -o microbench_issue
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

@@ -2,7 +2,7 @@
 // (64-bit canonical, ntt1024.h, vs redundant 24-bit limbs, ntt1024_l4.h), timed at the occupancy of
 // the bootstrap kernel (2 waves per SIMD, one 512-thread work-group per CU, LDS exchanges included);
 // (2) issue cost of further single VALU instructions at the same occupancy.
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -I../nufhe_amd/csrc microbench_l4.hip -o microbench_l4
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -I../nufhe_amd/csrc microbench_l4.hip -o microbench_l4
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

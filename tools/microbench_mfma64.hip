@@ -14,7 +14,7 @@
 //   m|i : two waves per SIMD, one MFMA-only, its partner v_add_u32-only
 // Output: shader cycles per MFMA (or per VALU instruction) per wave, the sustained clock, for 1 and 2 waves per SIMD.
 //
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 microbench_mfma64.hip -o microbench_mfma64
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 microbench_mfma64.hip -o microbench_mfma64
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

@@ -8,6 +8,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 asm = '/tmp/xfft.s'
 flags = sys.argv[1:]
 subprocess.check_call(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '--offload-arch=gfx950', '-S', '--cuda-device-only',
+                       '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
                        'kernels_xfft.hip', '-o', asm] + flags, cwd=os.path.join(ROOT, 'nufhe_amd', 'csrc'),
                       stderr=subprocess.DEVNULL)
 L = open(asm).read().split('\n')
