@@ -132,3 +132,15 @@ def test_the_flags_keep_packed_fp32_out_of_the_isa(tmp_path):
         subprocess.check_call(cmd + ['--cuda-device-only', '-S', str(src), '-o', str(out)], stderr=subprocess.DEVNULL)
         found[name] = bool(PACKED_FP32.search(out.read_text()))
     assert found == {'flags': False, 'plain': True}
+
+
+def test_build_compiles_what_is_already_built(monkeypatch):
+    """build() is the check that the sources compile: it runs the compiler on every unit, whatever objects are there."""
+    import __graft_entry__
+    run = []
+    monkeypatch.setattr(__graft_entry__.subprocess, 'check_call', lambda cmd, **kw: run.append(cmd))
+    __graft_entry__.build()
+    library = [cmd for cmd in run if any(str(w).endswith(os.path.join('nufhe_amd', 'csrc')) for w in cmd)]
+    assert len(library) == 1
+    text = subprocess.run(library[0] + ['-n'], text=True, check=True, capture_output=True).stdout
+    assert sum(' -c ' in l for l in text.split('\n')) == 5
