@@ -42,18 +42,20 @@ typedef int32_t i32;
 /* nufhe/transform/arithmetic.mako:78-462.                             */
 /* ------------------------------------------------------------------ */
 
-static inline u64 ff_mod(u64 x) { return x >= FF_P ? x - FF_P : x; } /* arithmetic.mako:164-194 */
+/* the corrections are masks, not branches: they are taken at random, and a wrong guess costs more than the whole product */
+static inline u64 ff_mask(int c) { return 0 - (u64)c; }
+
+static inline u64 ff_mod(u64 x) { return x - (FF_P & ff_mask(x >= FF_P)); } /* arithmetic.mako:164-194 */
 
 static inline u64 ff_add(u64 a, u64 b) /* arithmetic.mako:78-119; a,b < P */
 {
-    u128 s = (u128)a + b;
-    if (s >= FF_P) s -= FF_P;
-    return (u64)s;
+    u64 s = a + b; /* wrapped past 2^64, or at or above P: P too much either way */
+    return s - (FF_P & ff_mask((s < a) | (s >= FF_P)));
 }
 
 static inline u64 ff_sub(u64 a, u64 b) /* arithmetic.mako:122-161; a,b < P */
 {
-    return a >= b ? a - b : a + (FF_P - b);
+    return a - b + (FF_P & ff_mask(a < b));
 }
 
 static inline u64 ff_reduce128(u128 x)

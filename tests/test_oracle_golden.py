@@ -238,3 +238,15 @@ def test_fft_oracle_vs_reference(orc, golden):
     eq(res, golden['fft_extmul'])
     exact = orc.tgsw_external_mul(accum, orc.tlwe_transform_samples(tgsw), row)
     eq(golden['fft_extmul'], exact)
+
+
+def test_field_sums_at_every_border(orc):
+    """Sums, differences and the single reduction at the values where they wrap past 2^64, past P or below 0, all pairs
+    against Python integers."""
+    low = [0, 1, 2, 2**32 - 2, 2**32 - 1, 2**32, 2**32 + 1, 2**63 - 1, 2**63, P // 2, P // 2 + 1, P - 2**32, P - 2, P - 1]
+    a, b = numpy.array([(x, y) for x in low for y in low], numpy.uint64).T.copy()
+    eq(orc.ff_add(a, b), numpy.array([(x + y) % P for x in low for y in low], numpy.uint64))
+    eq(orc.ff_sub(a, b), numpy.array([(x - y) % P for x in low for y in low], numpy.uint64))
+    eq(orc.ff_mul(a, b), numpy.array([x * y % P for x in low for y in low], numpy.uint64))
+    high = low + [P, P + 1, 2**64 - 2, 2**64 - 1]
+    eq(orc.ff_mod(numpy.array(high, numpy.uint64)), numpy.array([x % P for x in high], numpy.uint64))
